@@ -8,9 +8,11 @@
 // The other operand of each product is split into two fp16 terms, hi = fp16(x) and lo = fp16(x - hi),
 // which together hold 22 bits of x; products and sums are in 32 bits, so the outputs keep the accuracy
 // of a 32-bit computation (one fp16 term alone would cost 2^-12 relative). Queries are first brought
-// to a power of two near 2^9 per row, probabilities carry a factor of 2^11 (2^-1 once a value scale of 2
-// and more was met), so that nothing overflows and the low terms keep clear of fp16's subnormal end: the
-// products of probabilities and scales are held to 2^-34 (2^-24) at the least.
+// to a power of two near 2^9 per row, probabilities carry a factor of 2^11, so that with scales below 2
+// nothing overflows, and the products of probabilities and scales are held to 2^-34 at the least. A tile with a
+// value scale of 2 or more has each block's products brought to the same place first, by the power of two
+// of the largest among them, and what they add up to brought back in 32 bits (where every tile is such a one,
+// 2000 rows behind none, 32 heads of size 64 over 8, take 88 us, else 58; 32 rows of 64 to 2048 11.0 and 9.6).
 //
 // A workgroup takes sets of 16 CT columns, a column being one (row, head) pair of one KV head: the
 // heads of a group for one row, or of several rows of a prompt chunk. The waves that share a set take its
@@ -57,8 +59,15 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 constexpr float kLog2E = 1.4426950408889634f;
 // The probabilities' power of two, and how far above the reference a score may rise (in powers of two)
 // before the reference follows it: most maxima after the first tile's stay within that, and following costs
-// a multiplication of every output. 2^(11 + 3) times a scale below 2, or 2^-1 times any scale, fit fp16.
-constexpr float kSmallShift = 11.0f, kBigShift = -1.0f, kRoom = 3.0f;
+// a multiplication of every output. 2^(11 + 3) times a scale below 2 fits fp16.
+constexpr float kShift = 11.0f, kRoom = 3.0f;
+
+// The power of two that brings a largest magnitude to [2^14, 2^15), within what has an inverse, and the inverse.
+__device__ __forceinline__ float to_fp16_range(float largest, float& inverse) {
+  const uint32_t up = min(268u - min(__float_as_uint(largest) >> 23, 255u), 253u);
+  inverse = __uint_as_float((254u - up) << 23);
+  return __uint_as_float(up << 23);
+}
 
 // 2^x, and 0 for -inf (the instruction; 1 ulp).
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -171,6 +180,21 @@ struct TileRing {
 // behind none, 32 heads of size 128 over 8: 96 us, one tile of columns a wave 110; 4000 rows 322 and 380).
 constexpr bool low_terms_in_lds(int nb, int ct) { return nb == 4 && ct == 2; }
 
+// Whether a tile holds a value scale of 2 or more, or one that is not finite (the top bit of its exponent is set),
+// among the positions below vis_hi: a lane takes the four of one block, a half-wave one of TILES tiles. The whole
+// wave agrees on it.
+template <int NB, int TILES, bool MASK>
+__device__ __forceinline__ bool wide_scales(const uint8_t* tile, uint32_t lane, int32_t pos0, int32_t vis_hi) {
+  const uint32_t which = TILES == 2 ? lane / 32 : 0, at = lane % (64 / TILES) % (8 * NB);  // (g 2 + s) NB + b
+  u32x2 d = *reinterpret_cast<const u32x2*>(tile + which * kv4_tile_bytes(32 * NB) + 1088 * NB + at * 8);
+  if constexpr (MASK) {
+    const int32_t left = vis_hi - pos0 - static_cast<int32_t>(which * kKv4Tile + at / (2 * NB) * 4 + at / NB % 2 * 16);
+    d[0] &= left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+    d[1] &= left >= 4 ? 0xffffffffu : left == 3 ? 0xffffu : 0u;
+  }
+  return __any(((d[0] | d[1]) & 0x40004000u) != 0);
+}
+
 // One wave's running softmax over its tiles, for 16 CT columns.
 template <int NB, int CT>
 struct WaveState {
@@ -183,12 +207,12 @@ struct WaveState {
   float ref[CT];           // what is subtracted in the exponent: top * colf - shift
   float sum[CT];           // this lane's part of the sum
   f32x4 o[CT][NB][2];
-  float shift;
 };
 
-template <int NB, int CT, bool MASK>
+// One tile. MASK: some column's row ends in it; WIDE: wide_scales.
+template <int NB, int CT, bool MASK, bool WIDE>
 __device__ __forceinline__ void tile_step(WaveState<NB, CT>& w, const CodeBits& bits, const uint8_t* tile, uint32_t lane,
-                                          const int32_t (&vis)[CT], int32_t vis_hi, int32_t pos0) {
+                                          const int32_t (&vis)[CT], int32_t pos0) {
   const uint32_t g = lane / 16;
   u32x2 kc[NB], kd[2 * NB], vc[NB], vd[2 * NB];
   lds_pairs<NB>(kc, tile + lane * (8 * NB));
@@ -221,19 +245,6 @@ __device__ __forceinline__ void tile_step(WaveState<NB, CT>& w, const CodeBits& 
   __builtin_amdgcn_sched_barrier(0);
   lds_pairs<NB>(vc, tile + 512 * NB + lane * (8 * NB));
   lds_pairs<2 * NB>(vd, tile + 1088 * NB + g * (16 * NB));
-  // A value scale of 2 or more (or not finite) has the top exponent bit set: such scales need the
-  // smaller power of two from here on. What no row sees does not count.
-  uint32_t big = 0;
-#pragma unroll
-  for (int i = 0; i < 2 * NB; ++i) {
-    if constexpr (MASK) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (pos0 + 16 * (i / NB) + r < vis_hi) big |= vd[i][r / 2] & (0x4000u << (16 * (r % 2)));
-    } else {
-      big |= vd[i][0] | vd[i][1];
-    }
-  }
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
     float m = -__builtin_inff();
@@ -247,10 +258,10 @@ __device__ __forceinline__ void tile_step(WaveState<NB, CT>& w, const CodeBits& 
     if (__builtin_expect(__any(m > w.limit[c]), 0)) {
       const float top = fmaxf(w.top[c], column_max(m));
       if (top != -__builtin_inff()) {
-        const float ref = __builtin_fmaf(top, w.colf[c], -w.shift);
+        const float ref = __builtin_fmaf(top, w.colf[c], -kShift);
         const float scale = w.top[c] == -__builtin_inff() ? 1.0f : exp2_fast(w.ref[c] - ref);
         w.top[c] = top;
-        w.limit[c] = top + (w.shift == kSmallShift ? kRoom / w.colf[c] : 0.0f);
+        w.limit[c] = top + kRoom / w.colf[c];
         w.ref[c] = ref;
         w.sum[c] *= scale;
 #pragma unroll
@@ -258,26 +269,6 @@ __device__ __forceinline__ void tile_step(WaveState<NB, CT>& w, const CodeBits& 
 #pragma unroll
           for (int h = 0; h < 2; ++h) w.o[c][b][h] *= scale;
       }
-    }
-  }
-  if (__builtin_expect(w.shift == kSmallShift && __any((big & 0x40004000u) != 0), 0)) {
-    // From here on there is no room above the reference: it goes to what this tile needs at once.
-    w.shift = kBigShift;
-#pragma unroll
-    for (int c = 0; c < CT; ++c) {
-      float m = w.top[c];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m = fmaxf(m, s[c][i]);
-      const float top = column_max(m);
-      const float ref = top == -__builtin_inff() ? w.ref[c] : __builtin_fmaf(top, w.colf[c], -kBigShift);
-      const float scale = w.top[c] == -__builtin_inff() ? 1.0f : exp2_fast(w.ref[c] - ref);
-      w.top[c] = w.limit[c] = top;
-      w.ref[c] = ref;
-      w.sum[c] *= scale;
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) w.o[c][b][h] *= scale;
     }
   }
   // Probabilities, and their sum.
@@ -292,11 +283,11 @@ __device__ __forceinline__ void tile_step(WaveState<NB, CT>& w, const CodeBits& 
   }
   // Outputs. A register of value codes holds positions r 0..3 in its bytes: (0, 2) and (1, 3) mask out
   // as pairs, which is the order that probabilities and scales take too: pair i is positions e and e + 2.
-  // Under the large power of two, probabilities are split into two fp16 terms once, and a product with a
+  // With scales below 2, probabilities are split into two fp16 terms once, and a product with a
   // scale, again in two terms, is three packed instructions a pair: hi = fp16(ph d), ph d - hi (exact),
   // and pl d added to it (a quarter less than two mixed multiply-adds a value, which run at half rate; 2000
-  // positions behind none, 32 heads of size 64 over 8: 58 us, was 65). Under the small one the smallest
-  // probabilities' terms are subnormal and scales may be large: there the products are split instead.
+  // positions behind none, 32 heads of size 64 over 8: 58 us, was 65). With larger ones the products are
+  // formed in 32 bits, and a block's are split where their own largest allows.
   uint32_t seen[CT][4];
   if constexpr (MASK) {
     // What lies past a row's own positions is not its, a NaN scale least of all.
@@ -308,7 +299,8 @@ __device__ __forceinline__ void tile_step(WaveState<NB, CT>& w, const CodeBits& 
         seen[c][i] = (at < vis[c] ? 0xffffu : 0u) | (at + 2 < vis[c] ? 0xffff0000u : 0u);
       }
   }
-  const auto add_values = [&](auto&& product) {
+  // add(c, b, the block's scales, its codes): a column's part of a block.
+  const auto each_block = [&](auto&& add) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const uint32_t w0 = vc[b][0], w1 = vc[b][1];
@@ -321,42 +313,56 @@ __device__ __forceinline__ void tile_step(WaveState<NB, CT>& w, const CodeBits& 
         d[i] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(dd[1], dd[0], i % 2 != 0 ? 0x07060302u : 0x05040100u));
       }
 #pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        half2_t hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          product(c, i, d[i], hi[i], lo[i]);
-          if constexpr (MASK) {
-            hi[i] = __builtin_bit_cast(half2_t, __builtin_bit_cast(uint32_t, hi[i]) & seen[c][i]);
-            lo[i] = __builtin_bit_cast(half2_t, __builtin_bit_cast(uint32_t, lo[i]) & seen[c][i]);
-          }
-        }
-        const half8_t phi = join8(hi[0], hi[1], hi[2], hi[3]), plo = join8(lo[0], lo[1], lo[2], lo[3]);
-        w.o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo16, plo, w.o[c][b][0], 0, 0, 0);
-        w.o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi16, plo, w.o[c][b][1], 0, 0, 0);
-        w.o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo16, phi, w.o[c][b][0], 0, 0, 0);
-        w.o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi16, phi, w.o[c][b][1], 0, 0, 0);
-      }
+      for (int c = 0; c < CT; ++c) add(c, b, d, lo16, hi16);
     }
   };
-  if (__builtin_expect(w.shift == kSmallShift, 1)) {
+  if constexpr (!WIDE) {
     half2_t ph[CT][4], pl[CT][4];
 #pragma unroll
     for (int c = 0; c < CT; ++c)
 #pragma unroll
       for (int i = 0; i < 4; ++i) split2(p[c][i / 2 * 4 + i % 2], p[c][i / 2 * 4 + i % 2 + 2], ph[c][i], pl[c][i]);
-    add_values([&](int c, int i, half2_t d, half2_t& hi, half2_t& lo) {
-      hi = ph[c][i] * d;
-      lo = __builtin_elementwise_fma(pl[c][i], d, __builtin_elementwise_fma(ph[c][i], d, -hi));
+    each_block([&](int c, int b, const half2_t (&d)[4], half8_t lo16, half8_t hi16) {
+      half2_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        hi[i] = ph[c][i] * d[i];
+        lo[i] = __builtin_elementwise_fma(pl[c][i], d[i], __builtin_elementwise_fma(ph[c][i], d[i], -hi[i]));
+        if constexpr (MASK) {
+          hi[i] = __builtin_bit_cast(half2_t, __builtin_bit_cast(uint32_t, hi[i]) & seen[c][i]);
+          lo[i] = __builtin_bit_cast(half2_t, __builtin_bit_cast(uint32_t, lo[i]) & seen[c][i]);
+        }
+      }
+      const half8_t phi = join8(hi[0], hi[1], hi[2], hi[3]), plo = join8(lo[0], lo[1], lo[2], lo[3]);
+      w.o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo16, plo, w.o[c][b][0], 0, 0, 0);
+      w.o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi16, plo, w.o[c][b][1], 0, 0, 0);
+      w.o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo16, phi, w.o[c][b][0], 0, 0, 0);
+      w.o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi16, phi, w.o[c][b][1], 0, 0, 0);
     });
   } else {
-    add_values([&](int c, int i, half2_t d, half2_t& hi, half2_t& lo) {
+    each_block([&](int c, int b, const half2_t (&d)[4], half8_t lo16, half8_t hi16) {
+      float x[8], most = 0.0f;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const float x = p[c][i / 2 * 4 + i % 2 + 2 * t], y = static_cast<float>(d[t]);
-        hi[t] = static_cast<_Float16>(__builtin_fmaf(x, y, 0.0f));
-        lo[t] = static_cast<_Float16>(__builtin_fmaf(x, y, -static_cast<float>(hi[t])));
+      for (int k = 0; k < 8; ++k) {
+        const int i = k / 2, at = i / 2 * 4 + i % 2 + k % 2 * 2;  // pair i's first and second
+        x[k] = p[c][at] * static_cast<float>(d[i][k % 2]);
+        if constexpr (MASK) x[k] = (seen[c][i] >> (16 * (k % 2)) & 1u) != 0 ? x[k] : 0.0f;
+        most = fmaxf(most, fabsf(x[k]));
       }
+      float inverse;
+      const float by = to_fp16_range(column_max(most), inverse);
+      half2_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) split2(x[2 * i] * by, x[2 * i + 1] * by, hi[i], lo[i]);
+      const half8_t phi = join8(hi[0], hi[1], hi[2], hi[3]), plo = join8(lo[0], lo[1], lo[2], lo[3]);
+      const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+      f32x4 even = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo16, plo, zero, 0, 0, 0);
+      f32x4 odd = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi16, plo, zero, 0, 0, 0);
+      even = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo16, phi, even, 0, 0, 0);
+      odd = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi16, phi, odd, 0, 0, 0);
+      w.o[c][b][0] += even * inverse;
+      w.o[c][b][1] += odd * inverse;
+      __builtin_amdgcn_sched_barrier(0);  // (one after another, in few registers)
     });
   }
 }
@@ -525,7 +531,6 @@ __global__ __launch_bounds__(W * 64, low_terms_in_lds(NB, CT) ? 2 : 1) void atte
 
   WaveState<NB, CT> w;
   w.low = reinterpret_cast<half8_t*>(lds + kRingBytes) + wave * (CT * NB * 64) + lane;
-  w.shift = kSmallShift;
   const float scale = fabsf(a.scale) * kLog2E;
   const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
@@ -574,11 +579,15 @@ __global__ __launch_bounds__(W * 64, low_terms_in_lds(NB, CT) ? 2 : 1) void atte
     }
     const uint32_t t = t0 + j * KS;
     const uint8_t* tile = slots + j % Ring::kDepth * Ring::kBytes;
-    const int32_t pos0 = static_cast<int32_t>(t * kKv4Tile + 4 * g);
-    if (static_cast<int32_t>((t + 1) * kKv4Tile) > vis_lo) {
-      tile_step<NB, CT, true>(w, bits, tile, lane, vis, vis_hi, pos0);
+    const int32_t first = static_cast<int32_t>(t * kKv4Tile), pos0 = first + static_cast<int32_t>(4 * g);
+    const bool mask = first + static_cast<int32_t>(kKv4Tile) > vis_lo;
+    const bool wide = mask ? wide_scales<NB, 1, true>(tile, lane, first, vis_hi) : wide_scales<NB, 1, false>(tile, lane, first, vis_hi);
+    if (__builtin_expect(wide, 0)) {
+      tile_step<NB, CT, true, true>(w, bits, tile, lane, vis, pos0);
+    } else if (mask) {
+      tile_step<NB, CT, true, false>(w, bits, tile, lane, vis, pos0);
     } else {
-      tile_step<NB, CT, false>(w, bits, tile, lane, vis, vis_hi, pos0);
+      tile_step<NB, CT, false, false>(w, bits, tile, lane, vis, pos0);
     }
   }
 
@@ -627,7 +636,6 @@ struct RowState {
   half4_t qhi[NS][2 * NB], qlo[NS][2 * NB];
   float colf[NS], top[NS], limit[NS], ref[NS], sum[NS];
   f32x4 o[NS][NB][2];
-  float shift;
 };
 
 // The largest over the 16 lanes with one l % 4.
@@ -639,11 +647,14 @@ __device__ __forceinline__ float head_max(float x) {
 
 __device__ __forceinline__ half4_t join4(half2_t a, half2_t b) { return half4_t{a[0], a[1], b[0], b[1]}; }
 
-// 64 positions: two tiles in LDS.
-template <int NB, int NS, bool MASK>
-__device__ __forceinline__ void row_step(RowState<NB, NS>& w, const CodeBits& bits, const uint8_t* tiles, uint32_t lane,
-                                         int32_t vis, int32_t pos0) {
+// 64 positions: two tiles in LDS, `at` bytes into the slots. MASK: the row ends in them; WIDE: wide_scales.
+template <int NB, int NS, bool MASK, bool WIDE>
+__device__ __forceinline__ void row_step(RowState<NB, NS>& w, const CodeBits& bits, const uint8_t* slots, uint32_t at,
+                                         uint32_t lane, int32_t vis, int32_t pos0) {
   constexpr uint32_t kTileBytes = kv4_tile_bytes(32 * NB);
+  // (Each form has its own beginning: what they share, ahead of the branch between them, holds a third more registers.)
+  asm volatile("" : "+s"(at));
+  const uint8_t* tiles = slots + at;
   // The lane's position as a row of the first product: its codes.
   uint32_t kc[4][NB];
   {
@@ -693,18 +704,6 @@ __device__ __forceinline__ void row_step(RowState<NB, NS>& w, const CodeBits& bi
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[n][r] = __builtin_fmaf(hi[n][r] + lo[n][r], half_of(kd[b], r), b == 0 ? 0.0f : s[n][r]);
   }
-  // A value scale of 2 or more asks for the smaller power of two, as in tile_step.
-  uint32_t big = 0;
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    if constexpr (MASK) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (pos0 + r < vis) big |= vd[b][r / 2] & (0x4000u << (16 * (r % 2)));
-    } else {
-      big |= vd[b][0] | vd[b][1];
-    }
-  }
 #pragma unroll
   for (int n = 0; n < NS; ++n) {
     if constexpr (MASK) {
@@ -713,14 +712,13 @@ __device__ __forceinline__ void row_step(RowState<NB, NS>& w, const CodeBits& bi
         if (pos0 + r >= vis) s[n][r] = -__builtin_inff();
     }
     const float m = fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3]));
-    const bool to_big = w.shift == kSmallShift && __any((big & 0x40004000u) != 0);
-    if (__builtin_expect(to_big || __any(m > w.limit[n]), 0)) {
-      const float top = fmaxf(w.top[n], head_max(m)), shift = to_big ? kBigShift : w.shift;
+    if (__builtin_expect(__any(m > w.limit[n]), 0)) {
+      const float top = fmaxf(w.top[n], head_max(m));
       // (a head without a score so far stays as it is)
-      const float ref = top == -__builtin_inff() ? w.ref[n] : __builtin_fmaf(top, w.colf[n], -shift);
+      const float ref = top == -__builtin_inff() ? w.ref[n] : __builtin_fmaf(top, w.colf[n], -kShift);
       const float scale = w.top[n] == -__builtin_inff() ? 1.0f : exp2_fast(w.ref[n] - ref);
       w.top[n] = top;
-      w.limit[n] = top + (shift == kSmallShift ? kRoom / w.colf[n] : 0.0f);
+      w.limit[n] = top + kRoom / w.colf[n];
       w.ref[n] = ref;
       w.sum[n] *= scale;
 #pragma unroll
@@ -731,47 +729,91 @@ __device__ __forceinline__ void row_step(RowState<NB, NS>& w, const CodeBits& bi
 #pragma unroll
           for (int k = 0; k < 2; ++k) w.o[n][b][k][r] *= of_head;
       }
-      if (n == NS - 1) w.shift = shift;
     }
   }
-  half4_t ph[NS][NB], pl[NS][NB];
+  float p[NS][4];
 #pragma unroll
   for (int n = 0; n < NS; ++n) {
-    float p[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) p[r] = exp2_fast(__builtin_fmaf(s[n][r], w.colf[n], -w.ref[n]));
-    w.sum[n] += (p[0] + p[1]) + (p[2] + p[3]);
-    constexpr int kOrder[4] = {0, 2, 1, 3};  // the order of a register of value codes
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int r = kOrder[k];
-        const float d = half_of(vd[b], r);
-        _Float16 hi = static_cast<_Float16>(__builtin_fmaf(p[r], d, 0.0f));
-        _Float16 lo = static_cast<_Float16>(__builtin_fmaf(p[r], d, -static_cast<float>(hi)));
-        if constexpr (MASK) {
-          if (pos0 + r >= vis) hi = lo = static_cast<_Float16>(0.0f);
-        }
-        ph[n][b][k] = hi;
-        pl[n][b][k] = lo;
-      }
-    }
+    for (int r = 0; r < 4; ++r) p[n][r] = exp2_fast(__builtin_fmaf(s[n][r], w.colf[n], -w.ref[n]));
+    w.sum[n] += (p[n][0] + p[n][1]) + (p[n][2] + p[n][3]);
   }
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
+  constexpr int kOrder[4] = {0, 2, 1, 3};  // the order of a register of value codes
+  // add(n, b, k, the codes): a set of heads' part of a block, over the k-th quarter of each 16 positions' products.
+  const auto each_block = [&](int b, auto&& add) {
     for_each_index<0, 4>([&]<int K>() {
       const uint32_t word = vc[K][b];
       const half4_t lo16 = join4(codes_low(bits, word), codes_low(bits, word >> 8));
       const half4_t hi16 = join4(codes_high(bits, word), codes_high(bits, word >> 8));
+      add.template operator()<K>(lo16, hi16);
+    });
+  };
+  if constexpr (!WIDE) {
+    half4_t ph[NS][NB], pl[NS][NB];
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = kOrder[k];
+          const float d = half_of(vd[b], r);
+          _Float16 hi = static_cast<_Float16>(__builtin_fmaf(p[n][r], d, 0.0f));
+          _Float16 lo = static_cast<_Float16>(__builtin_fmaf(p[n][r], d, -static_cast<float>(hi)));
+          if constexpr (MASK) {
+            if (pos0 + r >= vis) hi = lo = static_cast<_Float16>(0.0f);
+          }
+          ph[n][b][k] = hi;
+          pl[n][b][k] = lo;
+        }
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      each_block(b, [&]<int K>(half4_t lo16, half4_t hi16) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+          w.o[n][b][0] = __builtin_amdgcn_mfma_f32_4x4x4f16(pl[n][b], lo16, w.o[n][b][0], 2, K, 0);
+          w.o[n][b][1] = __builtin_amdgcn_mfma_f32_4x4x4f16(pl[n][b], hi16, w.o[n][b][1], 2, K, 0);
+          w.o[n][b][0] = __builtin_amdgcn_mfma_f32_4x4x4f16(ph[n][b], lo16, w.o[n][b][0], 2, K, 0);
+          w.o[n][b][1] = __builtin_amdgcn_mfma_f32_4x4x4f16(ph[n][b], hi16, w.o[n][b][1], 2, K, 0);
+        }
+      });
+    }
+  } else {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
-        w.o[n][b][0] = __builtin_amdgcn_mfma_f32_4x4x4f16(pl[n][b], lo16, w.o[n][b][0], 2, K, 0);
-        w.o[n][b][1] = __builtin_amdgcn_mfma_f32_4x4x4f16(pl[n][b], hi16, w.o[n][b][1], 2, K, 0);
-        w.o[n][b][0] = __builtin_amdgcn_mfma_f32_4x4x4f16(ph[n][b], lo16, w.o[n][b][0], 2, K, 0);
-        w.o[n][b][1] = __builtin_amdgcn_mfma_f32_4x4x4f16(ph[n][b], hi16, w.o[n][b][1], 2, K, 0);
+        float x[4], most = 0.0f, inverse;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = kOrder[k];
+          x[k] = p[n][r] * half_of(vd[b], r);
+          if constexpr (MASK) x[k] = pos0 + r < vis ? x[k] : 0.0f;
+          most = fmaxf(most, fabsf(x[k]));
+        }
+        const float by = to_fp16_range(head_max(most), inverse);
+        half2_t hi[2], lo[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) split2(x[2 * i] * by, x[2 * i + 1] * by, hi[i], lo[i]);
+        const half4_t ph = join4(hi[0], hi[1]), pl = join4(lo[0], lo[1]);
+        f32x4 even = {0.0f, 0.0f, 0.0f, 0.0f}, odd = {0.0f, 0.0f, 0.0f, 0.0f};
+        each_block(b, [&]<int K>(half4_t lo16, half4_t hi16) {
+          even = __builtin_amdgcn_mfma_f32_4x4x4f16(pl, lo16, even, 2, K, 0);
+          odd = __builtin_amdgcn_mfma_f32_4x4x4f16(pl, hi16, odd, 2, K, 0);
+          even = __builtin_amdgcn_mfma_f32_4x4x4f16(ph, lo16, even, 2, K, 0);
+          odd = __builtin_amdgcn_mfma_f32_4x4x4f16(ph, hi16, odd, 2, K, 0);
+        });
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float of_head = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(inverse), r));
+          w.o[n][b][0][r] += even[r] * of_head;
+          w.o[n][b][1][r] += odd[r] * of_head;
+        }
+        __builtin_amdgcn_sched_barrier(0);  // (one after another, in few registers)
       }
-    });
+    }
   }
 }
 
@@ -828,7 +870,6 @@ __global__ __launch_bounds__(W * 64) void attention_kv4_row_kernel(AttnKv4Args a
                                                 ((4 * c + lane % 4) * kDim + 16 * j + 4 * (lane / 16)) * 4);
 
   RowState<NB, NS> w;
-  w.shift = kSmallShift;
   const float scale = fabsf(a.scale) * kLog2E;
   const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
@@ -875,12 +916,16 @@ __global__ __launch_bounds__(W * 64) void attention_kv4_row_kernel(AttnKv4Args a
       wait_vm<0>();
     }
     const uint32_t step = step0 + j * W;
-    const uint8_t* at = slots + j % Ring::kDepth * Ring::kBytes;
-    const int32_t pos0 = static_cast<int32_t>(step * 64 + lane / 4 * 4);
-    if (static_cast<int32_t>((step + 1) * 64) > vis) {
-      row_step<NB, NS, true>(w, bits, at, lane, vis, pos0);
+    const uint32_t at = j % Ring::kDepth * Ring::kBytes;
+    const int32_t first = static_cast<int32_t>(step * 64), pos0 = first + static_cast<int32_t>(lane / 4 * 4);
+    const bool mask = first + 64 > vis;
+    const bool wide = mask ? wide_scales<NB, 2, true>(slots + at, lane, first, vis) : wide_scales<NB, 2, false>(slots + at, lane, first, vis);
+    if (__builtin_expect(wide, 0)) {
+      row_step<NB, NS, true, true>(w, bits, slots, at, lane, vis, pos0);
+    } else if (mask) {
+      row_step<NB, NS, true, false>(w, bits, slots, at, lane, vis, pos0);
     } else {
-      row_step<NB, NS, false>(w, bits, at, lane, vis, pos0);
+      row_step<NB, NS, false, false>(w, bits, slots, at, lane, vis, pos0);
     }
   }
 
