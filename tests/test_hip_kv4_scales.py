@@ -8,11 +8,14 @@ from test_hip_kv4 import Attention
 
 pytestmark = pytest.mark.gpu
 
+# ln(2) / 8 in 32 bits, whose product with log2(e) in 32 bits is 1 / 8.
+SCALE = float(np.float32(np.log(2) / 8))
+
 
 def bounded(q, k, v, v_scales, scale):
-    """One row's heads in 64 bits and how far the kernel's may be off, for queries that fp16 holds exactly and
-    key scales that are powers of two: the products' sums of a block are then exact, and a score is off by
-    the roundings of its blocks' sums (up to 8), of the factor and of the exponent's argument: within 2^-21 of
+    """One row's heads in 64 bits and how far the kernel's may be off, for queries that fp16 holds exactly,
+    key scales that are powers of two and SCALE: the products' sums of a block are then exact, and a score is off
+    by the roundings of its blocks' sums (up to 8), of SCALE and of the exponent's argument: within 2^-21 of
     the largest. A score off by e makes a probability off by e, in the numerator and in the sum. The
     exponential and the two fp16 terms of each product cost 2^-20, the 32-bit sums a rounding per step of 32
     positions and of the waves' and parts' joins (a quarter of the tiles at most falls to one wave, 64 for
@@ -49,12 +52,14 @@ def exact_queries(a, rng):
 
 
 def peak(a, cache, at, nats):
-    """Every head's score at a position, some nats above the others' mean: the heads share one query."""
+    """Two positions' scores some nats above the others' mean (every head's: they share one query), the second's a
+    little lower, so that its weight is no number of few bits."""
     a.q[:] = a.q[0, 0]
     (k, kd), _ = a.caches[cache]
-    kd[at] = 0.25
-    steps = int(np.clip(round(nats / (0.25 * a.scale * np.abs(a.q[0, 0]).sum())), -7, 7))
-    k[at] = np.where(a.q[0, 0] > 0, 8 + steps, 8 - steps)
+    kd[at] = kd[at + 21] = 0.5
+    steps = int(np.clip(round(nats / (0.5 * a.scale * np.abs(a.q[0, 0]).sum())), -6, 6))
+    k[at] = k[at + 21] = np.where(a.q[0, 0] > 0, 8 + steps, 8 - steps)
+    k[at + 21, :, :3] -= np.where(a.q[0, 0, :3] > 0, 1, -1).astype(np.int8).view(np.uint8)
 
 
 SHAPES = [(8, 2, 64), (8, 1, 128), (9, 3, 96), (4, 2, 256), (17, 1, 64), (6, 2, 192)]
@@ -64,7 +69,7 @@ SHAPES = [(8, 2, 64), (8, 1, 128), (9, 3, 96), (4, 2, 256), (17, 1, 64), (6, 2, 
 @pytest.mark.parametrize("large", [2.0, 300.0, 60000.0])
 @pytest.mark.parametrize("where", ["every", "first", "last", "some"])
 def test_small_scales_beside_a_large_one(n_head, n_kv, dim, large, where):
-    """One position has most of the weight and 4000 others share the rest; block 0 has a large scale at
+    """Two positions have most of the weight and 4000 others share the rest; block 0 has a large scale at
     every position, the first, the last or some, the others' are near 0.01. Rows of their own (split over
     workgroups, and not) and a chunk, of which only the last row sees the last position."""
     def change(a, rng):
@@ -75,10 +80,10 @@ def test_small_scales_beside_a_large_one(n_head, n_kv, dim, large, where):
             at = {"every": slice(None), "first": 0, "last": -1, "some": slice(7, None, 190)}[where]
             vd[at, :, 0] = np.float16(large)
             peak(a, i, len(vd) // 3, 10)
-    check(Attention([4001], n_head, n_kv, dim, seed=dim, change=change))
-    check(Attention([500, 33], n_head, n_kv, dim, seed=dim, change=change))
-    check(Attention([], n_head, n_kv, dim, chunk=(3, 3000), seed=dim, change=change))
-    check(Attention([], n_head, n_kv, dim, chunk=(40, 500), seed=dim, change=change))
+    check(Attention([4001], n_head, n_kv, dim, seed=dim, scale=SCALE, change=change))
+    check(Attention([500, 70], n_head, n_kv, dim, seed=dim, scale=SCALE, change=change))
+    check(Attention([], n_head, n_kv, dim, chunk=(3, 3000), seed=dim, scale=SCALE, change=change))
+    check(Attention([], n_head, n_kv, dim, chunk=(40, 500), seed=dim, scale=SCALE, change=change))
 
 
 @pytest.mark.parametrize("large", [2.0, 60000.0])
@@ -91,8 +96,8 @@ def test_large_scales_beside_small_ones_in_a_block(large):
                 vd[:] = (rng.uniform(0.01, 0.02, vd.shape)).astype(np.float16)
                 vd[len(vd) // 2] = np.float16(large)
                 peak(a, i, len(vd) // 2, nats)
-        check(Attention([3000], 8, 2, 64, seed=3, change=change))
-        check(Attention([], 8, 2, 64, chunk=(20, 2000), seed=4, change=change))
+        check(Attention([3000], 8, 2, 64, seed=3, scale=SCALE, change=change))
+        check(Attention([], 8, 2, 64, chunk=(20, 2000), seed=4, scale=SCALE, change=change))
 
 
 def test_earlier_rows_do_not_feel_a_later_rows_scale():
@@ -102,12 +107,12 @@ def test_earlier_rows_do_not_feel_a_later_rows_scale():
         for i, (_, (v, vd)) in enumerate(a.caches):
             vd[:] = (rng.uniform(0.01, 0.02, vd.shape)).astype(np.float16)
             peak(a, i, 100, 10)
-    plain = Attention([], 8, 2, 64, chunk=(16, 600), seed=5, change=change)
+    plain = Attention([], 8, 2, 64, chunk=(16, 600), seed=5, scale=SCALE, change=change)
 
     def larger(a, rng):
         change(a, rng)
         a.caches[0][1][1][-1] = np.float16(60000)
-    mixed = Attention([], 8, 2, 64, chunk=(16, 600), seed=5, change=larger)
+    mixed = Attention([], 8, 2, 64, chunk=(16, 600), seed=5, scale=SCALE, change=larger)
     out = mixed.run()
     check(mixed, out)
     check(plain, out, rows=range(15))
