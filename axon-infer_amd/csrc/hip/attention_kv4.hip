@@ -7,8 +7,10 @@
 // sum in 32 bits. For values the scale goes on the probability: out_b = sum_p (P_p d_v(p, b)) (c - 8).
 // The other operand of each product is split into two fp16 terms, hi = fp16(x) and lo = fp16(x - hi),
 // which together hold 22 bits of x; products and sums are in 32 bits, so the outputs keep the accuracy
-// of a 32-bit computation (one fp16 term alone would cost 2^-12 relative). Queries are first brought
-// to a power of two near 2^9 per row, probabilities carry a factor of 2^11, so that with scales below 2
+// of a 32-bit computation (one fp16 term alone would cost 2^-12 relative). Queries are first multiplied by
+// the mantissa of scale log2(e) and brought to a power of two near 2^9 per row, so that what is left of the
+// factor from a product's sum to the exponent is a power of two, and a score and its reference are compared
+// exactly however large they are. Probabilities carry a factor of 2^11, so that with scales below 2
 // nothing overflows, and the products of probabilities and scales are held to 2^-34 at the least. A tile with a
 // value scale of 2 or more has each block's products brought to the same place first, by the power of two
 // of the largest among them, and what they add up to brought back in 32 bits (where every tile is such a one,
@@ -61,6 +63,44 @@ constexpr float kLog2E = 1.4426950408889634f;
 // before the reference follows it: most maxima after the first tile's stay within that, and following costs
 // a multiplication of every output. 2^(11 + 3) times a scale below 2 fits fp16.
 constexpr float kShift = 11.0f, kRoom = 3.0f;
+
+// What a column's largest score so far sets: `ref`, which is subtracted in the exponent, and `limit`, the score above
+// which both are set anew. `factor` is a power of two, so t, the score in powers of two, is exact, and the reference
+// is t less kShift: the largest probability is 2^kShift. Where 32 bits do not hold that number (t from 2^24 on; the
+// nearest they hold would leave fp16's range from 2^25 on) it is t less 8, or t: all scores are whole multiples of a
+// power of two there, probabilities whole powers of two, and what they lose of their room below is not used.
+struct Reference {
+  float ref, limit;
+  __device__ __forceinline__ Reference(float top, float factor) {
+    const float t = top * factor;
+    ref = t - kShift;
+    limit = __builtin_fmaf(kRoom, __uint_as_float((254u << 23) - __float_as_uint(factor)), top);
+    if (__builtin_expect(fabsf((t - ref) - kShift) > 0.5f, 0)) {
+      ref = t - 8.0f;
+      if (t - ref > 8.5f) ref = t;
+      limit = top;
+    }
+  }
+};
+
+// What brings the queries of a head to 2^9 and more, their largest magnitude being `top`: first a power of two, then
+// a mantissa; and the power of two that the scores are left to be multiplied by.
+struct QueryScale {
+  float power, mantissa, factor;
+  // A query as it is split: rounded to 32 bits (split2).
+  __device__ __forceinline__ float operator()(float q) const {
+    float x = q * power * mantissa;
+    asm("" : "+v"(x));
+    return x;
+  }
+};
+__device__ __forceinline__ QueryScale query_scale(float top, float scale) {
+  const uint32_t up = min(263u - min(__float_as_uint(top) >> 23, 255u), 253u);
+  const float by = scale * kLog2E;
+  const int32_t left = __builtin_amdgcn_frexp_expf(by) + 127 - static_cast<int32_t>(up);
+  return QueryScale{__uint_as_float(up << 23), __builtin_amdgcn_frexp_mantf(by),
+                    __uint_as_float(static_cast<uint32_t>(min(max(left, -126), 127) + 127) << 23)};
+}
 
 // The power of two that brings a largest magnitude to [2^14, 2^15), within what has an inverse, and the inverse.
 __device__ __forceinline__ float to_fp16_range(float largest, float& inverse) {
@@ -118,7 +158,8 @@ __device__ __forceinline__ half2_t codes_high(const CodeBits& k, uint32_t w) {
   return __builtin_elementwise_fma(__builtin_bit_cast(half2_t, x), m, c);
 }
 // x and y as two fp16 terms each: hi the nearest, lo the nearest to the rest (the difference is one
-// mixed instruction, which the compiler makes two of).
+// mixed instruction, which the compiler makes two of). x and y are no products that round: the conversion would be
+// joined with the product, whose own rounding can part from that of the number it is in 32 bits.
 __device__ __forceinline__ void split2(float x, float y, half2_t& hi, half2_t& lo) {
   hi = half2_t{static_cast<_Float16>(x), static_cast<_Float16>(y)};
   float a, b;
@@ -201,10 +242,10 @@ struct WaveState {
   static constexpr bool kLowInLds = low_terms_in_lds(NB, CT);
   half8_t qhi[CT][NB], qlo[kLowInLds ? 1 : CT][kLowInLds ? 1 : NB];
   half8_t* low;            // the lane's of the first block, where they are in LDS: a block's are 64 apart
-  float colf[CT];          // score in powers of two per unit of the integer product
+  float colf[CT];          // score in powers of two per unit of the integer product: a power of two
   float top[CT];           // the reference, in those units: the maximum when it last moved
   float limit[CT];         // scores above it move the reference
-  float ref[CT];           // what is subtracted in the exponent: top * colf - shift
+  float ref[CT];           // what is subtracted in the exponent
   float sum[CT];           // this lane's part of the sum
   f32x4 o[CT][NB][2];
 };
@@ -258,11 +299,11 @@ __device__ __forceinline__ void tile_step(WaveState<NB, CT>& w, const CodeBits& 
     if (__builtin_expect(__any(m > w.limit[c]), 0)) {
       const float top = fmaxf(w.top[c], column_max(m));
       if (top != -__builtin_inff()) {
-        const float ref = __builtin_fmaf(top, w.colf[c], -kShift);
-        const float scale = w.top[c] == -__builtin_inff() ? 1.0f : exp2_fast(w.ref[c] - ref);
+        const Reference to(top, w.colf[c]);
+        const float scale = w.top[c] == -__builtin_inff() ? 1.0f : exp2_fast(w.ref[c] - to.ref);
         w.top[c] = top;
-        w.limit[c] = top + kRoom / w.colf[c];
-        w.ref[c] = ref;
+        w.limit[c] = to.limit;
+        w.ref[c] = to.ref;
         w.sum[c] *= scale;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
@@ -531,8 +572,6 @@ __global__ __launch_bounds__(W * 64, low_terms_in_lds(NB, CT) ? 2 : 1) void atte
 
   WaveState<NB, CT> w;
   w.low = reinterpret_cast<half8_t*>(lds + kRingBytes) + wave * (CT * NB * 64) + lane;
-  const float scale = fabsf(a.scale) * kLog2E;
-  const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
     float top = 0.0f;
@@ -540,16 +579,13 @@ __global__ __launch_bounds__(W * 64, low_terms_in_lds(NB, CT) ? 2 : 1) void atte
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int t = 0; t < 8; ++t) top = fmaxf(top, fabsf(x[c][b][t / 4][t % 4]));
-    // The power of two that brings the column's largest query value to [2^9, 2^10).
-    top = column_max(top);
-    const uint32_t up = min(263u - min(__float_as_uint(top) >> 23, 255u), 253u);
-    const float by = sign * __uint_as_float(up << 23);
-    w.colf[c] = fmaxf(scale * __uint_as_float((254u - up) << 23), 1.17549435e-38f);
+    const QueryScale by = query_scale(column_max(top), a.scale);
+    w.colf[c] = by.factor;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       half2_t hi[4], lo[4];
 #pragma unroll
-      for (int t = 0; t < 8; t += 2) split2(x[c][b][t / 4][t % 4] * by, x[c][b][t / 4][t % 4 + 1] * by, hi[t / 2], lo[t / 2]);
+      for (int t = 0; t < 8; t += 2) split2(by(x[c][b][t / 4][t % 4]), by(x[c][b][t / 4][t % 4 + 1]), hi[t / 2], lo[t / 2]);
       w.qhi[c][b] = join8(hi[0], hi[1], hi[2], hi[3]);
       const half8_t qlo = join8(lo[0], lo[1], lo[2], lo[3]);
       if constexpr (low_terms_in_lds(NB, CT)) w.low[(c * NB + b) * 64] = qlo;
@@ -715,10 +751,11 @@ __device__ __forceinline__ void row_step(RowState<NB, NS>& w, const CodeBits& bi
     if (__builtin_expect(__any(m > w.limit[n]), 0)) {
       const float top = fmaxf(w.top[n], head_max(m));
       // (a head without a score so far stays as it is)
-      const float ref = top == -__builtin_inff() ? w.ref[n] : __builtin_fmaf(top, w.colf[n], -kShift);
+      const Reference to(top, w.colf[n]);
+      const float ref = top == -__builtin_inff() ? w.ref[n] : to.ref;
       const float scale = w.top[n] == -__builtin_inff() ? 1.0f : exp2_fast(w.ref[n] - ref);
       w.top[n] = top;
-      w.limit[n] = top + kRoom / w.colf[n];
+      w.limit[n] = to.limit;
       w.ref[n] = ref;
       w.sum[n] *= scale;
 #pragma unroll
@@ -870,8 +907,6 @@ __global__ __launch_bounds__(W * 64) void attention_kv4_row_kernel(AttnKv4Args a
                                                 ((4 * c + lane % 4) * kDim + 16 * j + 4 * (lane / 16)) * 4);
 
   RowState<NB, NS> w;
-  const float scale = fabsf(a.scale) * kLog2E;
-  const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
   for (int c = 0; c < NS; ++c) {
     float top = 0.0f;
@@ -879,15 +914,13 @@ __global__ __launch_bounds__(W * 64) void attention_kv4_row_kernel(AttnKv4Args a
     for (int j = 0; j < 2 * NB; ++j)
 #pragma unroll
       for (int t = 0; t < 4; ++t) top = fmaxf(top, fabsf(x[c][j][t]));
-    top = column_max(top);
-    const uint32_t up = min(263u - min(__float_as_uint(top) >> 23, 255u), 253u);
-    const float by = sign * __uint_as_float(up << 23);
-    w.colf[c] = fmaxf(scale * __uint_as_float((254u - up) << 23), 1.17549435e-38f);
+    const QueryScale by = query_scale(column_max(top), a.scale);
+    w.colf[c] = by.factor;
 #pragma unroll
     for (int j = 0; j < 2 * NB; ++j) {
       half2_t hi[2], lo[2];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) split2(x[c][j][2 * t] * by, x[c][j][2 * t + 1] * by, hi[t], lo[t]);
+      for (int t = 0; t < 2; ++t) split2(by(x[c][j][2 * t]), by(x[c][j][2 * t + 1]), hi[t], lo[t]);
       w.qhi[c][j] = join4(hi[0], hi[1]);
       w.qlo[c][j] = join4(lo[0], lo[1]);
     }

@@ -1,0 +1,68 @@
+"""Attention over a 4-bit cache at the ends of what its arguments allow: scores far above the exponent's usual
+range, blocks that are not numbers far below the maximum, offsets of a chunk's rows, sizes of a launch."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import axon_hip as H
+import kv4
+from test_hip_kv4 import Attention, addr, put
+
+gpu = pytest.mark.gpu
+
+# Heads and rows that take each kernel: single rows (whole and split), single rows of large groups or heads, chunks.
+FORMS = [dict(lengths=[300], n_head=8, n_kv=2, dim=64), dict(lengths=[3000], n_head=8, n_kv=1, dim=128),
+         dict(lengths=[2500, 40], n_head=17, n_kv=1, dim=64), dict(lengths=[300, 9], n_head=4, n_kv=2, dim=256),
+         dict(lengths=[33], n_head=8, n_kv=2, dim=64, chunk=(30, 270)), dict(lengths=[], n_head=8, n_kv=2, dim=64, chunk=(4, 3000)),
+         dict(lengths=[], n_head=256, n_kv=64, dim=32, chunk=(130, 0)), dict(lengths=[], n_head=8, n_kv=2, dim=192, chunk=(30, 70))]
+
+
+# ---------------------------------------------------------------------------------------------
+# Scores whose size leaves 32 bits no fraction
+
+@gpu
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("power", [20, 24, 25, 26, 27, 28, 30, 33, 60, 100])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_equal_scores_of_any_size(form, power, sign):
+    """Every position has the same key, so every weight is the same, and 32 bits give every position the same
+    score, however large: the mean of the values, to the rounding of a sum of that many products (2^-20
+    of the products' magnitudes and the joins' share besides)."""
+    def change(a, rng):
+        a.q[:] = np.float32(2.0 ** power) * rng.choice([1, 1.25, 1.5], a.q.shape) * sign
+        for (k, kd), _ in a.caches:
+            k[:] = 13
+            kd[:] = np.float16(1)
+    a = Attention(**form, seed=power, change=change)
+    out = a.run()
+    for r in range(a.rows):
+        n = a.vis[r]
+        v = kv4.dequantize(*a.caches[a.of[r]][1])[:n]
+        group = a.n_head // a.n_kv
+        want = np.repeat(v.mean(0), group, 0)
+        bound = np.repeat(np.abs(v).mean(0), group, 0) * (2.0 ** -20 + (n / 32 + 64) * 2.0 ** -24) + n * 8 * 2.0 ** -34
+        assert np.all(np.abs(out[r] - want) <= bound), (r, n)
+
+
+@gpu
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("power", [10, 20, 25, 26, 27, 28, 30, 33, 60, 100])
+def test_the_largest_score_of_any_size(form, power):
+    """One position's score is twice the largest of the others, and then some hundred above: its values alone
+    are the output. It is neither first nor last, so that some waves begin with others."""
+    def change(a, rng):
+        a.q[:] = np.float32(2.0 ** power) * rng.choice([1, 1.25, 1.5], a.q.shape)
+        for (k, kd), _ in a.caches:
+            kd[:] = np.float16(1)
+            k[:] = rng.integers(8, 11, (len(k), a.n_kv, 1))
+            k[len(k) // 3] = 15
+    a = Attention(**form, seed=power, change=change)
+    out = a.run()
+    for r in range(a.rows):
+        n, seq = a.vis[r], a.of[r]
+        at = len(a.caches[seq][0][0]) // 3
+        if at >= n:
+            continue
+        want = np.repeat(kv4.dequantize(*a.caches[seq][1])[at], a.n_head // a.n_kv, 0)
+        assert np.all(np.abs(out[r] - want) <= np.abs(want) * 2.0 ** -20), (r, n)
