@@ -1052,24 +1052,18 @@ __global__ __launch_bounds__(256) void attention_kv4_join_kernel(AttnKv4Args a, 
   const float all = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   const float f = ref == none ? 0.0f : exp2_fast(ref - all);
   if (tid < n) factor[tid] = f;
-  float total = f == 0.0f ? 0.0f : f * sum;
+  float total = f * sum;  // (of a part too far below to count too: a NaN in it does)
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
   if (lane == 0) sums[tid / 64] = total;
   __syncthreads();
   float o = 0.0f;
   if (set < per) {
-    // (a part without positions holds nothing)
 #pragma unroll
-    for (uint32_t i = 0; i < kEarly; ++i) {
-      const float k = set + i * per < n ? factor[set + i * per] : 0.0f;
-      o += k != 0.0f ? k * early[i] : 0.0f;
-    }
+    for (uint32_t i = 0; i < kEarly; ++i)
+      if (set + i * per < n) o += factor[set + i * per] * early[i];
 #pragma unroll 4
-    for (uint32_t s = set + kEarly * per; s < n; s += per) {
-      const float k = factor[s];
-      if (k != 0.0f) o += k * part[s * stride + d];
-    }
+    for (uint32_t s = set + kEarly * per; s < n; s += per) o += factor[s] * part[s * stride + d];
   }
   acc[tid] = o;
   __syncthreads();

@@ -66,3 +66,33 @@ def test_the_largest_score_of_any_size(form, power):
             continue
         want = np.repeat(kv4.dequantize(*a.caches[seq][1])[at], a.n_head // a.n_kv, 0)
         assert np.all(np.abs(out[r] - want) <= np.abs(want) * 2.0 ** -20), (r, n)
+
+
+# ---------------------------------------------------------------------------------------------
+# Blocks held as NaN, far below the maximum
+
+@gpu
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("which", ["key", "value"])
+def test_a_block_that_is_not_a_number_is_felt_at_any_weight(form, which):
+    """One position outweighs the rest by more than 32 bits can say, and a block of another, in a tile far from
+    it, is held as NaN: the rows that see it give NaN (a key's in its head's outputs, a value's in its
+    block's), whether the positions are split over workgroups or not, and everything else is a number."""
+    def change(a, rng):
+        a.q[:] = 4
+        for i, ((k, kd), (v, vd)) in enumerate(a.caches):
+            kd[:] = np.float16(1)
+            k[:] = rng.integers(6, 9, k.shape)
+            k[0] = 15
+            bad = kd if which == "key" else vd
+            bad[2 * len(bad) // 3, -1, 0] = np.nan
+    a = Attention(**form, seed=1, change=change)
+    out = a.run()
+    group, felt = a.n_head // a.n_kv, 0
+    for r in range(a.rows):
+        sees = a.vis[r] > 2 * len(a.caches[a.of[r]][0][0]) // 3
+        felt += sees
+        want = np.zeros(out[r].shape, bool)
+        want[-group:, :a.dim if which == "key" else 32] = sees
+        assert np.array_equal(np.isnan(out[r]), want), (r, a.vis[r])
+    assert felt != 0
