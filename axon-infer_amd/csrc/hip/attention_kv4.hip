@@ -422,6 +422,7 @@ struct Kv4Plan {
   uint32_t col_tiles;   // 16-column tiles a wave
   uint32_t shared_by;   // waves that share a set of columns and its positions
   bool by_row;          // the kernel for single rows
+  bool chunk;           // the rows are one sequence's, the first row's
 };
 
 // Column `col` of a workgroup: its row behind the first and its head in the group.
@@ -561,7 +562,7 @@ __global__ __launch_bounds__(W * 64, low_terms_in_lds(NB, CT) ? 2 : 1) void atte
 
   // The first tiles start while the queries are prepared.
   Ring ring;
-  ring.base = static_cast<const uint8_t*>(a.cache) + (a.cache_off != nullptr ? a.cache_off[r0] : 0) + a.layer_off +
+  ring.base = static_cast<const uint8_t*>(a.cache) + (a.cache_off != nullptr ? a.cache_off[plan.chunk ? 0 : r0] : 0) + a.layer_off +
               static_cast<size_t>(h) * kv4_tiles(a.max_ctx) * Ring::kBytes;
   ring.lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(as_lds(lds))) + wave * Ring::kWaveBytes;
   ring.lane = lane;
@@ -1123,6 +1124,7 @@ Kv4Plan decode_plan(const AttnKv4Args& a, uint32_t row0, uint32_t n_rows) {
 Kv4Plan chunk_plan(const AttnKv4Args& a, uint32_t n_rows) {
   Kv4Plan p{};
   p.n_rows = n_rows;
+  p.chunk = true;
   p.waves = 4;
   const uint32_t group = a.n_head / a.n_kv;
   p.per_group = 65536 / group + (65536 % group != 0);

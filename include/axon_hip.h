@@ -351,13 +351,14 @@ int axon_hip_kv4_read_rows(const axon_hip_kv4_read_args* args, size_t n_rows);
 /* axon_hip_attention_rows over a 4-bit cache: row r attends over positions [0, n_vis[r]) of the
  * sequence at cache_off[r]; a row that sees none gets zeros, and an n_vis above max_vis counts as
  * max_vis. The first chunk_rows rows belong to one sequence (a prompt chunk; cache_off[0] is
- * theirs), which lets them share its tiles; every other row names its own. Outputs are computed in
- * 32 bits, with queries and products of weights and value scales as two fp16 terms: a query's value to
- * 2^-21 of itself or 2^-33 of the head's largest, a product to 2^-20 of itself or 2^-34 of the row's largest
- * weight (in a tile of 32 positions with a value scale of 2 or more: or 2^-39 of the block's largest product
- * there). A row's last bits depend on how many rows are computed together. scratch: axon_hip_attention_kv4_scratch_floats
- * floats (which serve any smaller max_vis too), or NULL when that is 0; calls that may run at the
- * same time need their own. out and the inputs do not overlap. */
+ * theirs, the entries of its other rows are not read), which lets them share its tiles; every other
+ * row names its own. Outputs are computed in 32 bits, with queries and products of weights and value
+ * scales as two fp16 terms: a query's value to 2^-21 of itself or 2^-33 of the head's largest, a
+ * product to 2^-20 of itself or 2^-34 of the row's largest weight (in a tile of 32 positions with a
+ * value scale of 2 or more: or 2^-39 of the block's largest product there). A row's last bits depend
+ * on how many rows are computed together. scratch: axon_hip_attention_kv4_scratch_floats floats
+ * (which serve any smaller max_vis too), or NULL when that is 0; calls that may run at the same time
+ * need their own. out and the inputs do not overlap. */
 typedef struct {
   const float* q;           /* [rows][q_stride], n_head heads of head_dim */
   float* out;               /* [rows][out_stride] */

@@ -96,3 +96,22 @@ def test_a_block_that_is_not_a_number_is_felt_at_any_weight(form, which):
         want[-group:, :a.dim if which == "key" else 32] = sees
         assert np.array_equal(np.isnan(out[r]), want), (r, a.vis[r])
     assert felt != 0
+
+
+# ---------------------------------------------------------------------------------------------
+# A chunk's sequence
+
+@gpu
+@pytest.mark.parametrize("form", [dict(n_head=8, n_kv=2, dim=64, chunk=(300, 20)), dict(n_head=8, n_kv=2, dim=64, chunk=(6, 3000)),
+                                  dict(n_head=40, n_kv=1, dim=32, chunk=(20, 5)), dict(n_head=256, n_kv=64, dim=32, chunk=(130, 0))])
+def test_a_chunk_goes_by_the_first_rows_offset(form):
+    """Entries 1 to chunk_rows - 1 of cache_off are not read: they name another sequence here. The rows behind
+    the chunk go by their own."""
+    a = Attention([50, 7], seed=12, **form)
+    args = a.args()
+    off = np.array([i * a.slot for i in a.of], np.int64)
+    off[1:a.chunk_rows] = a.slot
+    entries = put(off)
+    args.cache_off = entries.ptr
+    H.call("attention_kv4", addr(args), a.rows)
+    a.check(a.got())
