@@ -1149,23 +1149,19 @@ int launched(const AttnKv4Args& a, const Kv4Plan& p) {
   return check_launch("attention_kv4 join");
 }
 
-int check_blocks(size_t blocks) {
-  return blocks > 0x7fffffffu ? fail(kInvalidArgument, "attention_kv4: %zu workgroups", blocks) : static_cast<int>(kOk);
+size_t workgroups(const AttnKv4Args& a, const Kv4Plan& p) {
+  return ceil_div(p.n_rows, p.block_rows) * a.n_kv * p.col_blocks * p.splits;
 }
 
 template <int NB, int CT, int KS, int W>
 int run(const AttnKv4Args& a, const Kv4Plan& p) {
-  const size_t blocks = ceil_div(p.n_rows, p.block_rows) * a.n_kv * p.col_blocks * p.splits;
-  if (const int rc = check_blocks(blocks); rc != kOk) return rc;
-  hipLaunchKernelGGL((attention_kv4_kernel<NB, CT, KS, W>), dim3(static_cast<uint32_t>(blocks)), dim3(W * 64), 0, stream(), a, p);
+  hipLaunchKernelGGL((attention_kv4_kernel<NB, CT, KS, W>), dim3(static_cast<uint32_t>(workgroups(a, p))), dim3(W * 64), 0, stream(), a, p);
   return launched(a, p);
 }
 
 template <int NB, int NS, int W>
 int run_rows(const AttnKv4Args& a, const Kv4Plan& p) {
-  const size_t blocks = static_cast<size_t>(p.n_rows) * a.n_kv * p.splits;
-  if (const int rc = check_blocks(blocks); rc != kOk) return rc;
-  hipLaunchKernelGGL((attention_kv4_row_kernel<NB, NS, W>), dim3(static_cast<uint32_t>(blocks)), dim3(W * 64), 0, stream(), a, p);
+  hipLaunchKernelGGL((attention_kv4_row_kernel<NB, NS, W>), dim3(static_cast<uint32_t>(workgroups(a, p))), dim3(W * 64), 0, stream(), a, p);
   return launched(a, p);
 }
 
@@ -1206,6 +1202,14 @@ size_t attention_kv4_scratch_floats(const AttnKv4Args& a, uint32_t n_rows) {
   if (a.chunk_rows != 0) floats = plan_floats(a, chunk_plan(a, std::min(a.chunk_rows, n_rows)));
   if (n_rows > a.chunk_rows) floats = std::max(floats, plan_floats(a, decode_plan(a, a.chunk_rows, n_rows - a.chunk_rows)));
   return floats;
+}
+
+// (Of either part, before the first is launched.)
+int attention_kv4_check_size(const AttnKv4Args& a, uint32_t n_rows) {
+  size_t most = 0;
+  if (a.chunk_rows != 0) most = workgroups(a, chunk_plan(a, a.chunk_rows));
+  if (n_rows > a.chunk_rows) most = std::max(most, workgroups(a, decode_plan(a, a.chunk_rows, n_rows - a.chunk_rows)));
+  return launch_fits("attention_kv4", most, 512, 1);
 }
 
 int attention_kv4_launch(const AttnKv4Args& a, uint32_t n_rows) {

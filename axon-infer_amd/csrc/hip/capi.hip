@@ -849,6 +849,7 @@ int axon_hip_rope_rows_kv4(const axon_hip_rope_rows_args* args, size_t max_ctx, 
   if (a.q != nullptr && (a.n_head == 0 || a.n_head > 65536)) return fail(kInvalidArgument, "rope_rows_kv4: %u heads", a.n_head);
   if (n_rows > 1 && (a.k_stride < a.n_kv * a.head_dim || (a.q != nullptr && a.q_stride < a.n_head * a.head_dim)))
     return fail(kInvalidArgument, "rope_rows_kv4: row strides %u, %u", a.q_stride, a.k_stride);
+  if (const int rc = rope_rows_kv4_check_size(a, n_rows); rc != kOk) return rc;
   AXON_READY();
   return rope_rows_kv4_launch(a, static_cast<uint32_t>(max_ctx), static_cast<uint32_t>(n_rows));
 }
@@ -861,6 +862,7 @@ int axon_hip_kv4_read_rows(const axon_hip_kv4_read_args* args, size_t n_rows) {
   if (const int rc = kv4_check("kv4_read_rows", a.cache, a.layer_off, a.n_kv, a.head_dim, a.max_ctx, n_rows); rc != kOk) return rc;
   if (a.k == nullptr && a.v == nullptr) return fail(kInvalidArgument, "kv4_read_rows: no output");
   if (n_rows > 1 && a.stride < a.n_kv * a.head_dim) return fail(kInvalidArgument, "kv4_read_rows: stride %u", a.stride);
+  if (const int rc = kv4_read_check_size(a, n_rows); rc != kOk) return rc;
   AXON_READY();
   return kv4_read_launch(a, static_cast<uint32_t>(n_rows));
 }
@@ -891,6 +893,7 @@ int axon_hip_attention_kv4(const axon_hip_attention_kv4_args* args, size_t n_row
   if (a.q == nullptr || a.out == nullptr) return fail(kInvalidArgument, "attention_kv4: q and out are required");
   if (n_rows > 1 && (a.q_stride < a.n_head * a.head_dim || a.out_stride < a.n_head * a.head_dim))
     return fail(kInvalidArgument, "attention_kv4: row strides %u, %u", a.q_stride, a.out_stride);
+  if (const int rc = attention_kv4_check_size(a, static_cast<uint32_t>(n_rows)); rc != kOk) return rc;
   if (a.scratch == nullptr && attention_kv4_scratch_floats(a, static_cast<uint32_t>(n_rows)) != 0)
     return fail(kInvalidArgument, "attention_kv4: scratch is required for this shape");
   AXON_READY();

@@ -50,9 +50,16 @@ constexpr uint32_t kv4_scale_half(uint32_t nb, uint32_t p, uint32_t b) {
   return ((p % 16 / 4 * 2 + p / 16) * nb + b) * 4 + p % 4;
 }
 
+// What a launch can take: fewer than 2^32 threads along x, 65535 workgroups along y.
+inline int launch_fits(const char* what, size_t x, size_t threads, size_t y) {
+  if (x > 0xffffffffu / threads || y > 65535) return fail(kInvalidArgument, "%s: %zu by %zu workgroups of %zu threads", what, x, y, threads);
+  return kOk;
+}
+
 // Rotates (rope_rows' arithmetic) and quantizes new rows into a 4-bit cache: a.cache_off and
 // a.k_layer_off in bytes.
 int rope_rows_kv4_launch(const RopeRowsArgs& a, uint32_t max_ctx, uint32_t n_rows);
+int rope_rows_kv4_check_size(const RopeRowsArgs& a, size_t n_rows);
 
 struct Kv4ReadArgs {
   const void* cache;
@@ -66,6 +73,7 @@ struct Kv4ReadArgs {
   uint32_t stride;
 };
 int kv4_read_launch(const Kv4ReadArgs& a, uint32_t n_rows);
+int kv4_read_check_size(const Kv4ReadArgs& a, size_t n_rows);
 
 struct AttnKv4Args {
   const float* q;
@@ -84,6 +92,7 @@ struct AttnKv4Args {
   void* outq;                // Q8_0 blocks [rows][n_head * head_dim / 32], or null
 };
 int attention_kv4_launch(const AttnKv4Args& a, uint32_t n_rows);
+int attention_kv4_check_size(const AttnKv4Args& a, uint32_t n_rows);
 size_t attention_kv4_scratch_floats(const AttnKv4Args& a, uint32_t n_rows);
 
 }  // namespace axon_hip

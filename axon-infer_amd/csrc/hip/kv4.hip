@@ -182,23 +182,32 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4ReadArgs a) {
   out[static_cast<size_t>(r) * a.stride + e] = d * (static_cast<float>(code & 15u) - 8.0f);
 }
 
+// Workgroups of a row that store, and that turn its query.
+uint32_t store_groups_of(const RopeRowsArgs& a) { return static_cast<uint32_t>(ceil_div(2 * a.n_kv * (a.head_dim / kQK), 8)); }
+uint32_t query_groups_of(const RopeRowsArgs& a) {
+  const bool turn = a.q != nullptr && (a.rotary_dim != 0 || a.bq != nullptr);
+  return turn ? static_cast<uint32_t>(ceil_div(static_cast<size_t>(a.n_head) * (a.head_dim / 2), 256)) : 0;
+}
+uint32_t read_groups_of(const Kv4ReadArgs& a) { return static_cast<uint32_t>(ceil_div(2 * static_cast<size_t>(a.n_kv) * a.head_dim, 256)); }
+
 }  // namespace
+
+int rope_rows_kv4_check_size(const RopeRowsArgs& a, size_t n_rows) {
+  return launch_fits("rope_rows_kv4", n_rows, 256, store_groups_of(a) + query_groups_of(a));
+}
+int kv4_read_check_size(const Kv4ReadArgs& a, size_t n_rows) { return launch_fits("kv4_read_rows", n_rows, 256, read_groups_of(a)); }
 
 int rope_rows_kv4_launch(const RopeRowsArgs& a, uint32_t max_ctx, uint32_t n_rows) {
   if (n_rows == 0) return kOk;
-  const uint32_t blocks = 2 * a.n_kv * (a.head_dim / kQK);
-  const uint32_t store_groups = static_cast<uint32_t>(ceil_div(blocks, 8));
-  const bool turn_q = a.q != nullptr && (a.rotary_dim != 0 || a.bq != nullptr);
-  const uint32_t q_groups = turn_q ? static_cast<uint32_t>(ceil_div(static_cast<size_t>(a.n_head) * (a.head_dim / 2), 256)) : 0;
-  hipLaunchKernelGGL(rope_rows_kv4_kernel, dim3(n_rows, store_groups + q_groups), dim3(256), 0, stream(), a, max_ctx,
+  const uint32_t store_groups = store_groups_of(a);
+  hipLaunchKernelGGL(rope_rows_kv4_kernel, dim3(n_rows, store_groups + query_groups_of(a)), dim3(256), 0, stream(), a, max_ctx,
                      store_groups);
   return check_launch("rope_rows_kv4");
 }
 
 int kv4_read_launch(const Kv4ReadArgs& a, uint32_t n_rows) {
   if (n_rows == 0) return kOk;
-  const uint32_t groups = static_cast<uint32_t>(ceil_div(2 * static_cast<size_t>(a.n_kv) * a.head_dim, 256));
-  hipLaunchKernelGGL(kv4_read_kernel, dim3(n_rows, groups), dim3(256), 0, stream(), a);
+  hipLaunchKernelGGL(kv4_read_kernel, dim3(n_rows, read_groups_of(a)), dim3(256), 0, stream(), a);
   return check_launch("kv4_read_rows");
 }
 

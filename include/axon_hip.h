@@ -323,7 +323,9 @@ size_t axon_hip_attention_scratch_floats(const axon_hip_attention_rows_args* arg
  *   value scales   the same.
  * Offsets into such a cache (cache_off, layer_off) are in BYTES and multiples of 16, its base is
  * 16-byte aligned, and max_ctx is at most 2^24. What is past the visible positions is never used,
- * whatever it holds. */
+ * whatever it holds. A call takes what a launch can: writes and reads fewer than 2^24 rows, and
+ * n_kv * head_dim / 128 + n_head * head_dim / 512 up to 65535; attention fewer than 2^23 pairs of a row
+ * and a KV head (of 16 heads of its group). */
 /* Bytes of one layer of one sequence, keys and values; 0 for sizes that are not supported. */
 size_t axon_hip_kv4_layer_bytes(size_t n_kv, size_t head_dim, size_t max_ctx);
 /* axon_hip_rope_rows whose k and v rows go into a 4-bit cache of max_ctx positions (args->cache,

@@ -115,3 +115,32 @@ def test_a_chunk_goes_by_the_first_rows_offset(form):
     args.cache_off = entries.ptr
     H.call("attention_kv4", addr(args), a.rows)
     a.check(a.got())
+
+
+# ---------------------------------------------------------------------------------------------
+# Sizes that no launch can take are refused as arguments, before any device is asked for
+
+def test_sizes_past_a_launch_are_refused():
+    def refuse(name, a, *rest):
+        with pytest.raises(H.HipError, match="workgroups"):
+            H.call(name, addr(a), *rest)
+
+    for n_kv, n_head, dim, rows in ((65536, 0, 256, 2), (32768, 0, 256, 1), (2, 65536, 256, 1 << 24), (32767, 512, 256, 3), (2, 4, 64, 1 << 24)):
+        a = H.RopeRowsArgs()
+        a.k = a.v = a.cache = a.table = a.pos = 4096
+        a.q = 4096 if n_head else None
+        a.n_head, a.n_kv, a.head_dim, a.rotary_dim = n_head, n_kv, dim, 32
+        a.q_stride, a.k_stride = n_head * dim, n_kv * dim
+        refuse("rope_rows_kv4", a, 64, rows)
+    for n_kv, dim, rows in ((65536, 256, 2), (32768, 256, 1), (2, 64, 1 << 24), (1, 32, (1 << 31) - 1)):
+        b = H.Kv4ReadArgs()
+        b.cache = b.k = b.v = b.pos = 4096
+        b.n_kv, b.head_dim, b.max_ctx, b.stride = n_kv, dim, 64, n_kv * dim
+        refuse("kv4_read_rows", b, rows)
+    for n_head, n_kv, rows, chunk in ((8, 8, 1 << 20, 0), (64, 1, 1 << 21, 0), (65536, 65536, 200, 0), (1, 1, 1 << 23, 0), (64, 64, 1 << 30, 1 << 30),
+                                      (8, 8, (1 << 20) + 16, 16), (8, 8, (1 << 27) + 1, 1 << 27)):
+        c = H.AttentionKv4Args()
+        c.q = c.out = c.cache = c.n_vis = c.scratch = 4096
+        c.n_head, c.n_kv, c.head_dim, c.max_ctx, c.max_vis, c.scale, c.chunk_rows = n_head, n_kv, 32, 64, 64, 0.125, chunk
+        c.q_stride = c.out_stride = n_head * 32
+        refuse("attention_kv4", c, rows)
