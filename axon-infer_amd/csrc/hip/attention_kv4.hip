@@ -684,14 +684,14 @@ __device__ __forceinline__ float head_max(float x) {
 
 __device__ __forceinline__ half4_t join4(half2_t a, half2_t b) { return half4_t{a[0], a[1], b[0], b[1]}; }
 
-// 64 positions: two tiles in LDS, `at` bytes into the slots. MASK: the row ends in them; WIDE: wide_scales.
+// 64 positions: two tiles in LDS, in one of the slots. MASK: the row ends in them; WIDE: wide_scales.
 template <int NB, int NS, bool MASK, bool WIDE>
-__device__ __forceinline__ void row_step(RowState<NB, NS>& w, const CodeBits& bits, const uint8_t* slots, uint32_t at,
+__device__ __forceinline__ void row_step(RowState<NB, NS>& w, const CodeBits& bits, const uint8_t* slots, uint32_t slot,
                                          uint32_t lane, int32_t vis, int32_t pos0) {
   constexpr uint32_t kTileBytes = kv4_tile_bytes(32 * NB);
   // (Each form has its own beginning: what they share, ahead of the branch between them, holds a third more registers.)
-  asm volatile("" : "+s"(at));
-  const uint8_t* tiles = slots + at;
+  asm volatile("" : "+s"(slot));
+  const uint8_t* tiles = slots + slot * (2 * kTileBytes);
   // The lane's position as a row of the first product: its codes.
   uint32_t kc[4][NB];
   {
@@ -950,16 +950,17 @@ __global__ __launch_bounds__(W * 64) void attention_kv4_row_kernel(AttnKv4Args a
       wait_vm<0>();
     }
     const uint32_t step = step0 + j * W;
-    const uint32_t at = j % Ring::kDepth * Ring::kBytes;
+    const uint32_t slot = j % Ring::kDepth;
+    const uint8_t* at = slots + slot * Ring::kBytes;
     const int32_t first = static_cast<int32_t>(step * 64), pos0 = first + static_cast<int32_t>(lane / 4 * 4);
     const bool mask = first + 64 > vis;
-    const bool wide = mask ? wide_scales<NB, 2, true>(slots + at, lane, first, vis) : wide_scales<NB, 2, false>(slots + at, lane, first, vis);
+    const bool wide = mask ? wide_scales<NB, 2, true>(at, lane, first, vis) : wide_scales<NB, 2, false>(at, lane, first, vis);
     if (__builtin_expect(wide, 0)) {
-      row_step<NB, NS, true, true>(w, bits, slots, at, lane, vis, pos0);
+      row_step<NB, NS, true, true>(w, bits, slots, slot, lane, vis, pos0);
     } else if (mask) {
-      row_step<NB, NS, true, false>(w, bits, slots, at, lane, vis, pos0);
+      row_step<NB, NS, true, false>(w, bits, slots, slot, lane, vis, pos0);
     } else {
-      row_step<NB, NS, false, false>(w, bits, slots, at, lane, vis, pos0);
+      row_step<NB, NS, false, false>(w, bits, slots, slot, lane, vis, pos0);
     }
   }
 
