@@ -144,3 +144,28 @@ def test_sizes_past_a_launch_are_refused():
         c.n_head, c.n_kv, c.head_dim, c.max_ctx, c.max_vis, c.scale, c.chunk_rows = n_head, n_kv, 32, 64, 64, 0.125, chunk
         c.q_stride = c.out_stride = n_head * 32
         refuse("attention_kv4", c, rows)
+
+
+# ---------------------------------------------------------------------------------------------
+# Nothing to see, and factors at their ends
+
+@gpu
+@pytest.mark.parametrize("form", FORMS)
+def test_no_row_sees_anything(form):
+    """max_vis 0 and every n_vis 0: zeros, and the cache is not read (its address is that of a buffer of one tile)."""
+    a = Attention(**form, seed=2)
+    args = a.args()
+    none, small = put(np.zeros(a.rows), np.int32), put(np.full(kv4.tile_bytes(a.dim), 255, np.uint8))
+    args.n_vis, args.max_vis, args.cache, args.cache_off = none.ptr, 0, small.ptr, None
+    H.call("attention_kv4", addr(args), a.rows)
+    assert np.all(a.got() == 0)
+
+
+@gpu
+@pytest.mark.parametrize("form", FORMS[:5])
+@pytest.mark.parametrize("scale,queries", [(0.0, 1.0), (-0.0, 1.0), (1e30, 1e-31), (-1e-30, 1e30), (1e-38, 1e37)])
+def test_scales_at_their_ends(form, scale, queries):
+    """A scale of zero weighs every position alike; one that only a query at the other end makes ordinary."""
+    def change(a, rng):
+        a.q *= np.float32(queries)
+    Attention(**form, seed=3, change=change, scale=float(np.float32(scale))).check()
