@@ -32,15 +32,16 @@
 // Few rows over long contexts are split further, one workgroup per run of positions, and a second
 // kernel joins the parts by their maxima.
 //
-// Bounds, as measured (heads over KV heads, head size; a large copy runs at 4.9 TB/s here, a large fp16 product at
-// 1.1 PFLOP/s):
-//   16 rows of 32768 positions (32/8, 128): 597 MB in 117 us, 5.1 TB/s: the codes' bytes;
-//   32 rows of 64 to 2048 (32/8, 64): 19 MB in 9.5 us: the longest row's steps, one workgroup a CU;
-//   1 row of 512 (9/3, 64): 4.6 us, the launch and one step after another;
+// Bounds, as measured (heads over KV heads, head size; a large copy runs at 4.9 TB/s here, reads alone at 6.3, a
+// large fp16 product at 1.1 PFLOP/s):
+//   16 rows of 32768 positions (32/8, 128): 597 MB in 114 us, 5.2 TB/s: the codes' bytes, and vector instructions,
+//   issued two thirds of the time;
+//   32 rows of 64 to 2048 (32/8, 64): 19 MB in 9.6 us: the longest row's steps, one workgroup a CU;
+//   1 row of 512 (9/3, 64): 4.8 us, the launch and one step after another;
 //   2000 rows behind none (32/8, 64): 16.4 GFLOP, twice that for the two terms, in 57 us: vector
 //   instructions are issued 61 % of the time (a wave's step of 32 positions by 32 columns is 230 of them:
 //   codes 72, scores' scales 32, maxima and exponentials 64, probabilities' terms 96) and the matrix cores busy
-//   20 %; 8192 rows 673 us, 408 TFLOP/s.
+//   20 %; 8192 rows 680 us, 404 TFLOP/s.
 #include "common.h"
 #include "kv4.h"
 
@@ -218,7 +219,7 @@ struct TileRing {
 };
 
 // Whether a wave keeps the queries' low terms in LDS, where registers would leave it alone on its SIMD (2000 rows
-// behind none, 32 heads of size 128 over 8: 96 us, one tile of columns a wave 110; 4000 rows 322 and 380).
+// behind none, 32 heads of size 128 over 8: 98 us, one tile of columns a wave 111; 4000 rows 324 and 386).
 constexpr bool low_terms_in_lds(int nb, int ct) { return nb == 4 && ct == 2; }
 
 // Whether a tile holds a value scale of 2 or more, or one that is not finite (the top bit of its exponent is set),
@@ -327,7 +328,7 @@ __device__ __forceinline__ void tile_step(WaveState<NB, CT>& w, const CodeBits& 
   // With scales below 2, probabilities are split into two fp16 terms once, and a product with a
   // scale, again in two terms, is three packed instructions a pair: hi = fp16(ph d), ph d - hi (exact),
   // and pl d added to it (a quarter less than two mixed multiply-adds a value, which run at half rate; 2000
-  // positions behind none, 32 heads of size 64 over 8: 58 us, was 65). With larger ones the products are
+  // positions behind none, 32 heads of size 64 over 8, take 57 us, with those 7 more). With larger ones the products are
   // formed in 32 bits, and a block's are split where their own largest allows.
   uint32_t seen[CT][4];
   if constexpr (MASK) {
@@ -890,8 +891,8 @@ __global__ __launch_bounds__(W * 64) void attention_kv4_row_kernel(AttnKv4Args a
   constexpr uint32_t kAhead = Ring::kDepth - 1;
   // The queries come first, through the slot that is filled last (zeros for heads past the group: nothing is
   // read there), then the first steps; a step there is not reads nothing. The queries are then waited for alone,
-  // and prepared while the first tiles are on their way (one row of 1024 positions
-  // 6.1 us, 6.8 with both waited for).
+  // and prepared while the first tiles are on their way (0.7 us less for a row of 1024 positions, now 5.9, than
+  // with both waited for).
   static_assert(kHeads * kDim * 4 <= Ring::kBytes, "the queries fit a slot");
   const RsrcWords qr = raw_buffer_words(a.q + static_cast<size_t>(r) * a.q_stride + h * group * kDim, group * kDim * 4);
 #pragma unroll
@@ -988,8 +989,8 @@ __global__ __launch_bounds__(W * 64) void attention_kv4_row_kernel(AttnKv4Args a
     }
   }
   __syncthreads();
-  // A thread an output (whole waves), its parts one after another: a row of 1024 positions 7.2 us, with
-  // eight outputs a thread, all of them one wave's, 7.6.
+  // A thread an output (whole waves), its parts one after another (0.4 us less for a row of 1024 positions than
+  // eight outputs a thread, all of them one wave's).
   for (uint32_t u = threadIdx.x; u < kHeads * kDim; u += W * 64) {
     const uint32_t col = u / kDim, d = u % kDim;
     float ref = -__builtin_inff(), sum = 0.0f, o = 0.0f;
@@ -1024,8 +1025,8 @@ __global__ __launch_bounds__(W * 64) void attention_kv4_row_kernel(AttnKv4Args a
 
 // Joins the parts of a (row, head) pair: grid (heads, rows). Threads first bring every part's
 // reference to its factor, then 256 / head_dim of them a value add the parts up. What a thread adds of the first
-// parts is on its way before it is known which parts there are (one row of 8192 positions 9.4 us, 10.6 with one
-// load behind another).
+// parts is on its way before it is known which parts there are (1.2 us less for one row of 8192 positions, now
+// 7.8, than with one load behind another).
 constexpr uint32_t kMaxSplits = 128;
 __global__ __launch_bounds__(256) void attention_kv4_join_kernel(AttnKv4Args a, Kv4Plan plan) {
   __shared__ float factor[kMaxSplits], red[4], sums[4], acc[256];
@@ -1083,9 +1084,9 @@ __global__ __launch_bounds__(256) void attention_kv4_join_kernel(AttnKv4Args a, 
 constexpr uint32_t chunk_tiles(uint32_t nb) { return nb <= 4 ? 2 : 1; }
 
 // Splits of rows' positions over workgroups of `waves` waves: for a workgroup a CU (two a CU cost more in
-// the joining than they gained: 32 rows of 4096 positions 17.0 us with 256, 22.0 with 512) while each wave keeps
-// two tiles, and none that does not spare every wave four tiles (one row of 1024 positions 7.6 us, in two parts
-// 9.1; 16 rows of 1536 9.5 and 11.0; one row of 2048 11.1 and in four parts 9.2; all 1.5 less since).
+// the joining than they gained: 32 rows of 4096 positions 16.0 us with 256, 21.3 with 512) while each wave keeps
+// two tiles, and none that does not spare every wave four tiles (one row of 1024 positions 5.9 us, in two parts
+// 7.3; 16 rows of 1536 7.7 and 9.4; one row of 2048 8.6 and in four parts 7.4; of 8192 25.2 and in sixteen 7.8).
 void split_positions(Kv4Plan& p, const AttnKv4Args& a, size_t items) {
   const uint32_t tiles = std::max(1u, kv4_tiles(a.max_vis));
   const uint32_t whole = p.by_row ? 2 * p.waves : p.waves;  // tiles of a step of all waves
@@ -1108,7 +1109,8 @@ Kv4Plan decode_plan(const AttnKv4Args& a, uint32_t row0, uint32_t n_rows) {
   p.by_row = group <= 8 && a.head_dim <= 128;
   p.col_blocks = static_cast<uint32_t>(ceil_div(group, 16));
   const uint32_t tiles = kv4_tiles(a.max_vis);
-  // Four waves up to two steps each (a step is a tile, of single rows two): 512 positions 4.8 us, with eight a fifth more.
+  // Four waves up to two steps each (a step is a tile, of single rows two): 256 rows of 512 positions 22.0 us, with
+  // eight 22.5; 64 rows 6.8 and 7.05; but one row 4.9 and 4.6.
   // (Eight waves of two sets of heads of size 128 would not have the registers.)
   p.waves = tiles <= (p.by_row ? 16u : 8u) || a.head_dim > 128 || (p.by_row && group > 4 && a.head_dim > 96) ? 4 : 8;
   split_positions(p, a, static_cast<size_t>(n_rows) * a.n_kv * p.col_blocks);
@@ -1116,12 +1118,14 @@ Kv4Plan decode_plan(const AttnKv4Args& a, uint32_t row0, uint32_t n_rows) {
 }
 
 // A chunk's rows. Two tiles of columns a wave share the codes' extraction, two waves on a set of columns
-// read a tile half as often as four; both need the columns to fill the chip. In us, 32 heads over 8 KV heads:
+// read a tile half as often as four; both need the columns to fill the chip. One tile and four waves are split over
+// positions, the others not. In us, from graph replays of 32 heads over 8 KV heads:
 //   size, rows behind positions    one tile, 4 waves   one, 2    two, 4    two, 2
-//   64, 128 behind 4000                         26.2     26.5      29.1
-//   64, 512 behind 0                            11.6     10.9      12.1
-//   64, 2000 behind 0                           68.7     64.6      74       58.2
-//   64 (14 heads over 2), 2000 behind 0         36.0     38.0      33.4
+//   64, 128 behind 4000                         28.9     49.3      38.9      69.1
+//   64, 512 behind 0                            11.2     10.9      11.8      14.6
+//   64, 2000 behind 0                           73.8     67.1      61.7      60.4
+//   64 (14 heads over 2), 2000 behind 0         37.1     38.7      33.0      39.2
+//   128, 2000 behind 0                         124      111       105        97.8
 Kv4Plan chunk_plan(const AttnKv4Args& a, uint32_t n_rows) {
   Kv4Plan p{};
   p.n_rows = n_rows;

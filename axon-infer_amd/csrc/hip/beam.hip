@@ -14,7 +14,7 @@
 // its count of better ones, so the order in which waves arrive does not matter.
 // The order is total: scores in 64 bits, then beam, then (in a beam) logit, then token.
 // Bound: the logits' bytes, 4 a candidate; the second kernel's latency comes on top. 8 groups of 8 beams
-// over 151936 tokens: 38.9 MB in 7.0 us (5.5 TB/s), then 7.0 us, of which about 1.8 read the parts and join
+// over 151936 tokens: 38.9 MB in 7.0 to 7.7 us (5.0 to 5.5 TB/s), then 6.9 us, of which about 1.8 read the parts and join
 // the sums, 1.1 find the bound, 1.4 read the chosen chunks and 1.8 gather and rank.
 //
 // Reorder. A thread holds one 16-byte piece of every slot of a group that changes: it loads all of them

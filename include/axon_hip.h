@@ -396,7 +396,7 @@ size_t axon_hip_attention_kv4_scratch_floats(const axon_hip_attention_kv4_args* 
  * beam with score -inf is dropped altogether, as are tokens masked with -inf). Where a group has
  * fewer than n_out candidates the rest has token -1, score -inf and parent 0.
  * 1 <= n_beams <= AXON_HIP_MAX_BEAMS, 1 <= n_out <= AXON_HIP_MAX_BEAM_OUT,
- * 1 <= n <= AXON_HIP_MAX_BEAM_VOCAB. work: device memory of axon_hip_beam_select_work_bytes bytes,
+ * 1 <= n <= AXON_HIP_MAX_BEAM_VOCAB, n_groups * n_beams <= 65535. work: device memory of axon_hip_beam_select_work_bytes bytes,
  * 8-byte aligned; calls that may run at the same time need their own. */
 typedef struct {
   const float* x;
@@ -419,7 +419,7 @@ int axon_hip_beam_select(const axon_hip_beam_select_args* args);
  * parent's; at most max_len, less than 2 GiB a region). F32 and F16 caches: regions are a layer's K
  * rows and V rows, a unit one row; 4-bit caches: regions are a layer's heads, a unit a tile of 32
  * positions. pool is 16-byte aligned; slot_off, region_stride and unit_bytes are multiples of 16,
- * or all of 4, or of 2. Slots do not overlap. */
+ * or all of 4, or of 2. Slots do not overlap. n_groups and n_regions are at most 65535. */
 typedef struct {
   void* pool;
   const int64_t* slot_off; /* device [n_groups * n_beams], bytes */
