@@ -14,7 +14,7 @@
 // nothing overflows, and the products of probabilities and scales are held to 2^-34 at the least. A tile with a
 // value scale of 2 or more has each block's products brought to the same place first, by the power of two
 // of the largest among them, and what they add up to brought back in 32 bits (where every tile is such a one,
-// 2000 rows behind none, 32 heads of size 64 over 8, take 88 us, else 58; 32 rows of 64 to 2048 11.0 and 9.6).
+// 2000 rows behind none, 32 heads of size 64 over 8, take 88 us, else 57; 32 rows of 64 to 2048 11.0 and 9.6).
 //
 // A workgroup takes sets of 16 CT columns, a column being one (row, head) pair of one KV head: the
 // heads of a group for one row, or of several rows of a prompt chunk. The waves that share a set take its
